@@ -460,13 +460,7 @@ __device__ __forceinline__ void team_forward_body(const RenderArgs& a)
                             s_res[buf][slot] = res;
                         }
                         if (hint_base && GENDR_TEAM_ABLATE != 3) {
-                            // the batch's pair hints leave through the scalar data cache (see render_forward_body)
-                            typedef unsigned u4s __attribute__((ext_vector_type(4)));
-                            const unsigned long long h_lo = __ballot(hint_bit0(hint));
-                            const unsigned long long h_hi = __ballot(hint_bit1(hint));
-                            u4s hv; hv.x = (unsigned)h_lo; hv.y = (unsigned)(h_lo >> 32); hv.z = (unsigned)h_hi; hv.w = (unsigned)(h_hi >> 32);
-                            PairHints* slot = hint_base + k;
-                            asm volatile("s_store_dwordx4 %0, %1, 0x0" :: "s"(hv), "s"(slot) : "memory");
+                            store_pair_hints(hint_base + k, hint, lane);
                             if (__ballot(hint_none(hint)) && lane == 0) atomicOr(a.control + (blockIdx.x & 7) * kCtlStride + kCtlHintFlag, 2);
                         }
                         // the next chunk's pairs (of this phase: a later phase's codes are not listed yet) are announced now
@@ -532,7 +526,6 @@ __device__ __forceinline__ void team_forward_body(const RenderArgs& a)
             }
         }
     }
-    if (hints_q && !folder) asm volatile("s_waitcnt lgkmcnt(0)\n s_dcache_wb\n s_waitcnt lgkmcnt(0)" ::: "memory");   // the hints' scalar stores reach the L2
 }
 
 // ---------------------------------------------------------------------------------------------

@@ -1,0 +1,22 @@
+"""Rules for the device code, read from the sources (no GPU needed): nothing writes through the scalar data cache."""
+import os
+import re
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+# scalar stores, scalar atomics, write-back and discard of the scalar cache
+SCALAR_WRITE = re.compile(r'\bs_(?:store_|buffer_store_|scratch_store_|atomic_|buffer_atomic_|dcache_wb|dcache_discard)')
+
+
+def device_sources():
+    """Every file of the tree a GPU program is built or started from, and the tools that read their listings."""
+    out = []
+    for top in ('gendr_amd', 'include', 'oracle', 'tools', 'profiles'):
+        for d, _, files in os.walk(os.path.join(ROOT, top)):
+            out += [os.path.join(d, f) for f in files if f.endswith(('.h', '.hip', '.cpp', '.c', '.inc', '.py', '.sh', '.s'))]
+    return sorted(out)
+
+
+def test_no_write_through_the_scalar_cache():
+    found = ['%s:%d' % (os.path.relpath(p, ROOT), i) for p in device_sources()
+             for i, line in enumerate(open(p, encoding='utf-8'), 1) if SCALAR_WRITE.search(line)]
+    assert not found, found

@@ -14,7 +14,7 @@ import sys
 def classify(op):
     if op.startswith(('s_waitcnt', 's_nop', 's_barrier', 's_sleep')):
         return 'wait/nop'
-    if op.startswith(('s_load', 's_buffer_load', 's_store', 's_dcache', 's_memtime')):
+    if op.startswith(('s_load', 's_buffer_load', 's_memtime')):
         return 'smem'
     if op.startswith(('s_cbranch', 's_branch', 's_endpgm', 's_setpc', 's_swappc', 's_getpc', 's_call')):
         return 'branch'
