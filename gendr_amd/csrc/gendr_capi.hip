@@ -327,6 +327,24 @@ Workspace workspace_layout(int B, int nf, int T, const gendr_params* p)
     return w;
 }
 
+// n 32-bit words of zeros by a kernel: a caller may capture every entry point in a HIP graph, and memset nodes of captured graphs have
+// given wrong results on replays after the first.  16-byte stores between a ragged head and tail (`p` need only be aligned to its words).
+__global__ __launch_bounds__(256) void zero_words_kernel(unsigned* p, long n)
+{
+    const long head = min(n, (long)((0u - (unsigned)(reinterpret_cast<unsigned long long>(p) >> 2)) & 3u));
+    const long quads = (n - head) >> 2;
+    const long i = (long)blockIdx.x * 256 + threadIdx.x, stride = (long)gridDim.x * 256;
+    uint4* q = reinterpret_cast<uint4*>(p + head);
+    for (long k = i; k < quads; k += stride) q[k] = make_uint4(0u, 0u, 0u, 0u);
+    const long rest = n - 4 * quads;                             // words before and behind the quads: at most six
+    if (i < rest) p[i < head ? i : 4 * quads + i] = 0u;
+}
+void zero_words(void* p, size_t n, hipStream_t s)
+{
+    const size_t blocks = std::min<size_t>((n / 4 + 255) / 256 + 1, 4096);      // (a grid-stride loop: 16 workgroups per CU)
+    hipLaunchKernelGGL(zero_words_kernel, dim3((unsigned)blocks), dim3(256), 0, s, static_cast<unsigned*>(p), (long)n);
+}
+
 // gendr_params::deterministic: one wavefront per (image, face), see render_backward_faces_body; the few faces with a large
 // cull box are cut into row bands (second launch) whose sums a third launch adds up in a fixed order.  Uses the scratch region
 // at the end of the workspace (the one part of it that gendr_backward writes).
@@ -343,7 +361,7 @@ int launch_deterministic_backward(RenderArgs& a, const void* workspace, int B, i
     a.det_count = reinterpret_cast<int*>(base + w.det_off);
     a.det_list = a.det_count + 64;
     a.det_partial = reinterpret_cast<float*>(base + w.det_off + align256((size_t)(kDetBigCap + 64) * sizeof(int)));
-    if (hipMemsetAsync(a.det_count, 0, sizeof(int), s) != hipSuccess) return GENDR_E_LAUNCH;
+    zero_words(a.det_count, 1, s);
     const int texm = texture_mode(p, T);
     const KernelEntry& k = pick_generic(p, texm, silhouette);
     hipLaunchKernelGGL(k.det, dim3((unsigned)blocks), dim3(kDetThreads), 0, s, a, boxes);
@@ -696,7 +714,7 @@ int gendr_silhouette_forward(const float* faces, float* alpha, void* workspace, 
     if ((long)B * nf > 0 && !faces) return GENDR_E_NULL;
     const int e = face_setup_impl(faces, faces /* never read in this texture mode */, workspace, B, nf, kSilT, p, stream, true);
     if (e != GENDR_OK) return e;
-    if (target && hipMemsetAsync(iou_sums, 0, (size_t)B * 2 * sizeof(float), (hipStream_t)stream) != hipSuccess) return GENDR_E_LAUNCH;
+    if (target) zero_words(iou_sums, (size_t)B * 2, (hipStream_t)stream);
     RenderArgs a;
     const int texm = fill_args(a, workspace, nullptr, B, nf, kSilT, p);
     a.rgba = alpha;
@@ -823,7 +841,7 @@ int gendr_selftest(int what, unsigned long long* report16, void* stream)
 {
     if (!report16) return GENDR_E_NULL;
     if (what < 0 || what > 6) return GENDR_E_SHAPE;
-    if (hipMemsetAsync(report16, 0, 16 * sizeof(unsigned long long), (hipStream_t)stream) != hipSuccess) return GENDR_E_LAUNCH;
+    zero_words(report16, 32, (hipStream_t)stream);
     hipLaunchKernelGGL(selftest_kernel, dim3(256 * 16), dim3(256), 0, (hipStream_t)stream, what, report16);
     return check_launch();
 }
@@ -1044,7 +1062,7 @@ int gendr_voxelize(const float* faces, int* voxels, void* workspace, int B, int 
     const bool in_lds = vs <= 64;
     if (!in_lds && !workspace) return GENDR_E_NULL;
     hipStream_t st = (hipStream_t)stream;
-    if (hipMemsetAsync(voxels, 0, (size_t)B * vs * vs * vs * sizeof(int), st) != hipSuccess) return GENDR_E_LAUNCH;
+    zero_words(voxels, (size_t)B * vs * vs * vs, st);
     if (nf > 0) {
         const int work = vs * vs > nf ? vs * vs : nf;
         hipLaunchKernelGGL(voxel_surface_kernel, dim3((work + kVoxSurfaceThreads - 1) / kVoxSurfaceThreads, 4, B),

@@ -124,6 +124,12 @@ def render_silhouette(face_vertices, image_size=256, dist_func='uniform', dist_s
     return SilhouetteFunction.apply(face_vertices, p)
 
 
+def view_sums(x):
+    """[B, S, S] -> [B].  torch cuts ONE large sum (a view of 512^2 and more) over several workgroups and clears their counters with a
+    memset, which a captured HIP graph must not hold: inside a capture the rows are summed first, a workgroup at most for each."""
+    return x.sum(2).sum(1) if torch.cuda.is_current_stream_capturing() else x.sum((1, 2))
+
+
 def silhouette_iou(face_vertices, target, image_size=256, dist_func='uniform', dist_scale=1e-2, dist_squared=False,
                    dist_shape=None, dist_shift=None, dist_eps=1e4, aggr_alpha_func='probabilistic',
                    aggr_alpha_t_conorm_p=None, near=1, far=100, return_alpha=False):
@@ -133,7 +139,7 @@ def silhouette_iou(face_vertices, target, image_size=256, dist_func='uniform', d
                 aggr_alpha_func, aggr_alpha_t_conorm_p, near, far)
     sums, alpha, tgt = SilhouetteIoUFunction.apply(face_vertices, target, p)     # tgt: the target on the render device, float32
     intersect = sums[:, 0]
-    union = tgt.sum((1, 2)) + sums[:, 1]
+    union = view_sums(tgt) + sums[:, 1]
     return (intersect, union, alpha) if return_alpha else (intersect, union)
 
 

@@ -74,9 +74,7 @@ class GenDR(nn.Module):
         in the forward kernel and the gradient formed in the backward kernel.  Without anti-aliasing only."""
         from .functional.silhouette import silhouette_iou_loss
         if self.anti_aliasing:
-            from .functional.silhouette import render_silhouette
+            from .functional.silhouette import view_sums
             a = self.silhouette(mesh)
-            dims = tuple(range(1, a.ndimension()))
-            inter = (a * target).sum(dims)
-            return (1. - inter / ((a + target - a * target).sum(dims) + eps)).mean()
+            return (1. - view_sums(a * target) / (view_sums(a + target - a * target) + eps)).mean()
         return silhouette_iou_loss(mesh.face_vertices, target, eps=eps, image_size=self.image_size, **self._silhouette_options())

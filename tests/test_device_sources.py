@@ -1,4 +1,5 @@
-"""Rules for the device code, read from the sources (no GPU needed): nothing writes through the scalar data cache."""
+"""Rules for the device code, read from the sources (no GPU needed): nothing writes through the scalar data cache; the entry points record
+no memset (a caller may capture them in a HIP graph)."""
 import os
 import re
 
@@ -19,4 +20,11 @@ def device_sources():
 def test_no_write_through_the_scalar_cache():
     found = ['%s:%d' % (os.path.relpath(p, ROOT), i) for p in device_sources()
              for i, line in enumerate(open(p, encoding='utf-8'), 1) if SCALAR_WRITE.search(line)]
+    assert not found, found
+
+
+def test_entry_points_record_no_memset():
+    csrc = os.path.join(ROOT, 'gendr_amd', 'csrc')
+    found = ['%s:%d' % (f, i) for f in sorted(os.listdir(csrc)) if f.endswith(('.h', '.hip', '.cpp'))
+             for i, line in enumerate(open(os.path.join(csrc, f), encoding='utf-8'), 1) if re.search(r'\b(?:hip|cuda)Memset', line)]
     assert not found, found
