@@ -445,7 +445,7 @@ def measure(args, wl, dist, dev):
         finally:
             gc.enable()
     if dist is not None:
-        t = torch.tensor([elapsed], dtype=torch.float64, device='cpu' if stub else dev)
+        t = torch.tensor([elapsed], dtype=torch.float64, device='cpu' if stub or dist.get_backend() == 'gloo' else dev)
         dist.all_reduce(t, op=dist.ReduceOp.MAX)
         elapsed = float(t.item())
     out = dict(elapsed=elapsed, launch=launch, fwd_ms=None, bwd_ms=None, n_events=len(events), coll_ms=None)

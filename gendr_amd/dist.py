@@ -5,7 +5,8 @@ independently (``kernel.cu:714,903``: ``bn = i / (is*is)``, no cross-batch term)
 only in callers whose loss couples views (all-gather of rendered views; shared-geometry
 optimisation such as ``experiments/opt_shape.py:86``: sum of the vertex gradient over ranks).
 ``torch.distributed`` with backend "nccl" is RCCL on ROCm (xGMI within a node); the same code runs on
-"gloo" for the CPU tests.
+"gloo" for the CPU tests.  gloo is handed host memory only: where its ranks hold device tensors (several ranks on one GPU, which RCCL
+refuses) they are copied to the host and back around the exchange -- its collectives on device tensors have hung there.
 """
 import torch
 import torch.distributed as dist
@@ -52,6 +53,15 @@ class _Timed:
         return False
 
 
+def _gloo(group):
+    return dist.get_backend(group) == 'gloo'
+
+
+def _staged(t, group):
+    """Whether ``t`` has to go through host memory (see the module's first lines).  The copies are synchronous."""
+    return t.device.type != 'cpu' and _gloo(group)
+
+
 def _check_equal_blocks(n_local, group):
     """all_gather_into_tensor / reduce_scatter_tensor need the same block size on every rank: unequal blocks hang
     or corrupt on NCCL / RCCL instead of failing.  One tiny all-reduce (min and max of the local size) and a host read on
@@ -63,7 +73,7 @@ def _check_equal_blocks(n_local, group):
         raise RuntimeError('gather_views: the equal-block check reads a value back on the host and cannot run inside a HIP graph capture; '
                            'callers that shard evenly pass assume_equal_blocks=True (bench.py does)')
     t = torch.tensor([n_local, -n_local], dtype=torch.int64)
-    if dist.get_backend(group) != 'gloo':
+    if not _gloo(group):
         t = t.cuda()
     dist.all_reduce(t, op=dist.ReduceOp.MAX, group=group)
     lo, hi = -int(t[1]), int(t[0])
@@ -115,6 +125,27 @@ def _algorithm(direct):
     return bool(direct)
 
 
+def _all_gather(out, x, group, direct):
+    if direct:
+        _direct_all_gather(out, x, group)
+    else:
+        dist.all_gather_into_tensor(out, x, group=group)
+
+
+def _reduce_scatter(grad, n, rank, group, direct):
+    """Rank ``rank``'s block of ``n`` views of the (contiguous) gradient's sum over ranks."""
+    if _gloo(group) and not direct:                    # gloo has no reduce_scatter: all-reduce a private copy and slice
+        total = grad.clone()                           # never reduce in place into autograd's own buffer
+        dist.all_reduce(total, group=group)
+        return total[rank * n:(rank + 1) * n].clone()
+    out = torch.empty((n,) + tuple(grad.shape[1:]), dtype=grad.dtype, device=grad.device)
+    if direct:
+        _direct_reduce_scatter(out, grad, group)
+    else:
+        dist.reduce_scatter_tensor(out, grad, group=group)
+    return out
+
+
 class _GatherViews(torch.autograd.Function):
     """All-gather of equally sized per-rank view blocks; backward = reduce-scatter of the gradient
     (each rank receives the sum over ranks of the gradient w.r.t. its own block)."""
@@ -129,10 +160,12 @@ class _GatherViews(torch.autograd.Function):
         x = x.contiguous()
         out = torch.empty((world * x.shape[0],) + tuple(x.shape[1:]), dtype=x.dtype, device=x.device)
         with _Timed(x):
-            if direct:
-                _direct_all_gather(out, x, group)
+            if _staged(x, group):
+                host = torch.empty_like(out, device='cpu')
+                _all_gather(host, x.cpu(), group, direct)
+                out.copy_(host)
             else:
-                dist.all_gather_into_tensor(out, x, group=group)
+                _all_gather(out, x, group, direct)
         return out
 
     @staticmethod
@@ -140,21 +173,12 @@ class _GatherViews(torch.autograd.Function):
         group = ctx.group
         world, rank = dist.get_world_size(group), dist.get_rank(group)
         n = grad.shape[0] // world
-        if ctx.direct:
-            grad = grad.contiguous()
-            out = torch.empty((n,) + tuple(grad.shape[1:]), dtype=grad.dtype, device=grad.device)
-            with _Timed(grad):
-                _direct_reduce_scatter(out, grad, group)
-            return out, None, None, None
-        if dist.get_backend(group) == 'gloo':          # gloo has no reduce_scatter: all-reduce a private copy and slice
-            total = grad.clone(memory_format=torch.contiguous_format)   # never reduce in place into autograd's own buffer
-            with _Timed(total):
-                dist.all_reduce(total, group=group)
-            return total[rank * n:(rank + 1) * n].clone(), None, None, None
         grad = grad.contiguous()
-        out = torch.empty((n,) + tuple(grad.shape[1:]), dtype=grad.dtype, device=grad.device)
         with _Timed(grad):
-            dist.reduce_scatter_tensor(out, grad, group=group)
+            if _staged(grad, group):
+                out = _reduce_scatter(grad.cpu(), n, rank, group, ctx.direct).to(grad.device)
+            else:
+                out = _reduce_scatter(grad, n, rank, group, ctx.direct)
         return out, None, None, None
 
 
@@ -175,5 +199,10 @@ def gather_views(images, group=None, assume_equal_blocks=False, direct=None):
 def sum_over_ranks(t, group=None):
     """In-place sum of a (small) tensor over ranks, e.g. the gradient of geometry shared by all views."""
     if dist.is_initialized() and dist.get_world_size(group) > 1:
-        dist.all_reduce(t, group=group)
+        if _staged(t, group):
+            host = t.cpu()
+            dist.all_reduce(host, group=group)
+            t.copy_(host)
+        else:
+            dist.all_reduce(t, group=group)
     return t
