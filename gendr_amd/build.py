@@ -33,7 +33,9 @@ def lib_path(variant="default"):
 SOURCES = ["gendr_capi.hip"]
 HEADERS = ["gendr_kernels.h", "gendr_team.h", "gendr_math.h", "gendr_project.h", "gendr_voxel.h", "gendr_texture.h", "gendr_light.h", os.path.join("compat", "gendr_f64.h"), os.path.join("..", "..", "include", "gendr_hip.h")]
 HIPCC_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-ffp-contract=off", "-fPIC", "-shared",
-               "-munsafe-fp-atomics", "-fno-slp-vectorize"]
+               "-munsafe-fp-atomics", "-fno-slp-vectorize",
+               # no packed float instructions (v_pk_add / mul / fma_f32): some of their forms have given wrong results on this chip
+               "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def _hipcc():

@@ -128,7 +128,8 @@ def build(verbose=False):
             assert translated and os.path.dirname(os.path.abspath(translated)) == tmp, translated
             co = os.path.join(REF_DIR, 'gendr_ref_%s.co' % name)
             cmd = [CLANG, '-x', 'hip', '--offload-arch=gfx950', '--cuda-device-only', '--no-gpu-bundle-output', '-O3',
-                   '-std=c++17', '-D__HIP_PLATFORM_AMD__=1', '-DUSE_ROCM=1', '-w'] + extra + inc + ['-c', translated, '-o', co]
+                   '-std=c++17', '-D__HIP_PLATFORM_AMD__=1', '-DUSE_ROCM=1', '-w',
+                   '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops'] + extra + inc + ['-c', translated, '-o', co]
             r = subprocess.run(cmd, capture_output=True, text=True)
             if r.returncode != 0:
                 raise RuntimeError('reference device code of %s did not compile:\n%s' % (f, r.stderr[-4000:]))

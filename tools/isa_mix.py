@@ -1,6 +1,6 @@
 """Instruction mix of the render kernels from the compiler's ISA listing.
 
-    hipcc --offload-arch=gfx950 -O3 -std=c++17 -ffp-contract=off -munsafe-fp-atomics -save-temps -c gendr_amd/csrc/gendr_capi.hip
+    hipcc --offload-arch=gfx950 -O3 -std=c++17 -ffp-contract=off -munsafe-fp-atomics -fno-slp-vectorize -Xclang -target-feature -Xclang -packed-fp32-ops -save-temps -c gendr_amd/csrc/gendr_capi.hip
     python tools/isa_mix.py gendr_capi-hip-amdgcn-amd-amdhsa-gfx950.s [substring of the kernel name ...]
 
 Static counts per kernel: f32 VALU, f64 VALU (incl. conversions to / from f64), transcendental (v_exp/log/rcp/rsq/sqrt/sin/cos),

@@ -1,7 +1,7 @@
 // Micro-benchmark: issue cost (SIMD cycles per wave-instruction sequence) of the division / sqrt / exp forms the pair
 // math can choose from.  Every lane runs ITER independent evaluations per form on 8 interleaved chains; the grid fills
 // the chip with 8 waves per SIMD, so the result is throughput, not latency.
-//   hipcc --offload-arch=gfx950 -O3 -ffp-contract=off tools/micro/opbench.hip -o tools/micro/bin/opbench
+//   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -ffp-contract=off tools/micro/opbench.hip -o tools/micro/bin/opbench
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cmath>

@@ -1,7 +1,7 @@
 // Where does the library's powf(x, 2.f) differ from the correctly rounded square x * x?  For every float x of [2^-20, 16]:
 // mismatches, and how close the exact square lies to a rounding midpoint in those cases (|x*x - RN(x*x)| / (ulp / 2): 1 = on the
 // midpoint).  Decides the margin of the fast form of GammaFamily::cdf's power (gendr_math.h).
-//   hipcc --offload-arch=gfx950 -O3 -ffp-contract=off tools/micro/pow2probe.hip -o tools/micro/bin/pow2probe
+//   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -ffp-contract=off tools/micro/pow2probe.hip -o tools/micro/bin/pow2probe
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cmath>

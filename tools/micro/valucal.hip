@@ -4,7 +4,7 @@
 //     SQ_ACTIVE_INST_VALU * 4 / (1024 SIMDs * kernel duration * 2.4 GHz)
 // reads for it is the factor the same expression over-reads by for every other kernel (clock below nominal under counters, the
 // counter's unit); tools/pmc_finalize.py divides by it.  SQ_THREAD_CYCLES_VALU / (64 SQ_ACTIVE_INST_VALU) must read 1.00 here.
-//   hipcc --offload-arch=gfx950 -O3 tools/micro/valucal.hip -o tools/micro/bin/valucal
+//   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops tools/micro/valucal.hip -o tools/micro/bin/valucal
 #include <hip/hip_runtime.h>
 #include <cstdio>
 
