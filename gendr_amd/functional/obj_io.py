@@ -242,7 +242,7 @@ def voxelization(faces, size, normalize=False):
     if faces.dim() != 4 or faces.shape[2:] != (3, 3):
         raise ValueError('faces must be [B, nf, 3, 3]; got %s' % (tuple(faces.shape),))
     size = int(size)
-    faces = faces.detach().to(torch.float32).clone()
+    faces = faces.detach().to(torch.float32).clone(memory_format=torch.contiguous_format)     # (a plain clone keeps a dense permuted layout)
     if not normalize:
         faces *= size
     B, nf = faces.shape[:2]
