@@ -200,9 +200,9 @@ def sum_over_ranks(t, group=None):
     """In-place sum of a (small) tensor over ranks, e.g. the gradient of geometry shared by all views."""
     if dist.is_initialized() and dist.get_world_size(group) > 1:
         if _staged(t, group):
-            host = t.cpu()
+            host = t.detach().cpu()
             dist.all_reduce(host, group=group)
-            t.copy_(host)
+            t.detach().copy_(host)                     # (a leaf that requires grad as well)
         else:
             dist.all_reduce(t, group=group)
     return t

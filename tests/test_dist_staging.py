@@ -51,11 +51,12 @@ def test_gather_views(handed, monkeypatch, backend, where, direct):
 
 
 @pytest.mark.parametrize("backend,where", [('gloo', 'cpu'), ('nccl', 'cuda')])
-def test_sum_over_ranks(handed, monkeypatch, backend, where):
+@pytest.mark.parametrize("leaf", [False, True])
+def test_sum_over_ranks(handed, monkeypatch, backend, where, leaf):
     from gendr_amd.dist import sum_over_ranks
     monkeypatch.setattr(dist, 'get_backend', lambda group=None: backend)
     with FakeTensorMode():
-        t = torch.empty(7, 3, device='cuda')
+        t = torch.empty(7, 3, device='cuda', requires_grad=leaf)
         assert sum_over_ranks(t) is t and t.device.type == 'cuda'
     assert handed == [where]
 
